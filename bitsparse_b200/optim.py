@@ -91,9 +91,15 @@ class Muon(torch.optim.Optimizer):
         p -= lr * (scale * orthogonalize(grad + momentum * buf) + weight_decay * p)
 
     (without ``nesterov``: orthogonalize(buf)), scale = sqrt(max(1, rows /
-    cols)).  Parameters of more dimensions are matrices of their first one by
-    the rest.  For a model's matrices; embeddings, norms and biases belong to
-    another optimiser.
+    cols)).  Parameters (bf16 or fp32) of more dimensions are matrices of their
+    first one by the rest.  For a model's matrices; embeddings, norms and biases
+    belong to another optimiser.
+
+    The state is fp32 whatever the parameters' type.  A bf16 parameter is the
+    rounding of a fp32 value, and what that rounding left is kept beside the
+    momentum (``remainder``): a decay or update far below a bf16 step adds up
+    over the steps.  Where someone else changed a parameter in between, its
+    remainder no longer belongs to it and is dropped.
     """
 
     def __init__(self, params: Iterable, lr: float = 0.02, momentum: float = 0.95,
@@ -110,38 +116,70 @@ class Muon(torch.optim.Optimizer):
                     raise ValueError("Muon steps matrices; a parameter has "
                                      f"{p.dim()} dimension(s)")
 
+    def load_state_dict(self, state_dict):
+        """The state is copied, in fp32: the base class would cast it to the
+        parameters' type."""
+        seen = []
+        hook = self.register_load_state_dict_pre_hook(lambda _, d: seen.append(d))
+        try:  # (the last hook of those that may have changed the dictionary)
+            super().load_state_dict(state_dict)
+        finally:
+            hook.remove()
+        state_dict = seen[-1]
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            for p, key in zip(group["params"], saved["params"]):
+                for name in ("momentum_buffer", "remainder"):
+                    value = state_dict["state"].get(key, {}).get(name)
+                    if value is not None:
+                        self.state[p][name] = value.to(p.device, torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        work = []  # (group, matrices of one shape and type)
         for group in self.param_groups:
             same: dict = {}
             for p in group["params"]:
                 if p.grad is not None and p.numel():
+                    if p.dtype not in (torch.bfloat16, torch.float32):
+                        raise TypeError(f"Muon steps bfloat16 or float32 parameters, not {p.dtype}")
                     rows = p.shape[0]
                     same.setdefault((rows, p.numel() // rows, p.dtype, p.device), []).append(p)
-            for (rows, cols, _, _), params in same.items():
-                self._step_shape(group, params, rows, cols)
+            work += [(group, params, key[0], key[1]) for key, params in same.items()]
+        for args in work:
+            self._step_shape(*args)
         return loss
+
+    def _states(self, params, name):
+        for p in params:
+            if name not in self.state[p]:
+                self.state[p][name] = torch.zeros_like(p, dtype=torch.float32)
+        return [self.state[p][name] for p in params]
 
     def _step_shape(self, group, params, rows, cols):
         momentum, lr = group["momentum"], group["lr"]
-        grads = [p.grad for p in params]
-        bufs = []
-        for p in params:
-            state = self.state[p]
-            if "momentum_buffer" not in state:
-                state["momentum_buffer"] = torch.zeros_like(p)
-            bufs.append(state["momentum_buffer"])
+        narrow = params[0].dtype != torch.float32
+        grads = [p.grad.float() for p in params]
+        bufs = self._states(params, "momentum_buffer")
         torch._foreach_mul_(bufs, momentum)
         torch._foreach_add_(bufs, grads)
         updates = torch._foreach_add(grads, bufs, alpha=momentum) if group["nesterov"] else bufs
         batch = torch.stack([u.reshape(rows, cols) for u in updates])
         o = orthogonalize(batch, steps=group["steps"], coefficients=group["coefficients"])
+        values = params
+        if narrow:  # the fp32 values that the parameters are the roundings of
+            values = self._states(params, "remainder")
+            torch._foreach_add_(values, params)
+            for p, v in zip(params, values):
+                v.copy_(torch.where(v.to(p.dtype) == p, v, p))
         if group["weight_decay"]:
-            torch._foreach_mul_(params, 1 - lr * group["weight_decay"])
+            torch._foreach_mul_(values, 1 - lr * group["weight_decay"])
         scale = max(1.0, rows / cols) ** 0.5
-        steps = [v.view(p.shape).to(p.dtype) for p, v in zip(params, o.unbind())]
-        torch._foreach_add_(params, steps, alpha=-lr * scale)
+        steps = [v.view(p.shape).float() for p, v in zip(params, o.unbind())]
+        torch._foreach_add_(values, steps, alpha=-lr * scale)
+        if narrow:  # rounded once; the difference is exact
+            torch._foreach_copy_(params, values)
+            torch._foreach_sub_(values, params)

@@ -609,15 +609,25 @@ __global__ void __launch_bounds__(kThreadsB) logprobs_bwd_kernel(const LogprobPa
   const float m = P.stats[2 * row], log_s = P.stats[2 * row + 1];
   const bool dead = m == -INFINITY;
   const float k = P.rcp_t * kLog2e, shift = dead ? 0.f : -log_s * kLog2e;
-  // d = p (a + b (x - m)) + (column is the target) at
-  const float a = none || dead ? 0.f : -P.rcp_t * (gl + gh * (P.ent[row] - log_s));
+  // d = p (a + b (x - m)), at the target's column + at
+  const float ah = none || dead ? 0.f : -P.rcp_t * (gh * (P.ent[row] - log_s));
   const float b = none || dead ? 0.f : -P.rcp_t * P.rcp_t * gh, at = gl * P.rcp_t;
+  const float a = none || dead ? 0.f : ah - at;
   // (a row with NaN has m NaN and with it a; so NaN need not be looked for)
   const float a_ = m == m ? a : m;
+  // Where p is near 1, at (1 - p) as at - at p would keep the rounding of p
+  // alone (1e-3 of it at log p = -2e-5); -expm1(log p) has the digits of 1 - p.
+  // (Only there: few rows wait for it.)  One thread of a row comes here.
+  auto at_target = [&]() {
+    if (none || dead) return none ? 0.f : at;
+    const float d = fmaxf(Vec<T>::get(x + target) - m, kFloor), p = ex2(fmaf(d, k, shift));
+    const float logprob = fmaf(d, P.rcp_t, -log_s);
+    return fmaf(at, logprob > -0.5f ? -expm1f(logprob) : 1.f - p, p * fmaf(b, d, ah));
+  };
   auto grad = [&](float v, int c) {
     const float d = fmaxf(v - m, kFloor);
-    const float g = none || dead ? 0.f : ex2(fmaf(d, k, shift)) * fmaf(b, d, a_);
-    return c == target ? g + at : g;
+    if (c == target) return at_target();
+    return none || dead ? 0.f : ex2(fmaf(d, k, shift)) * fmaf(b, d, a_);
   };
   const float2 minus_m = both(-m), k2 = both(k), shift2 = both(shift), a2 = both(a_), b2 = both(b);
   const int V = (int)P.V;
@@ -647,9 +657,10 @@ __global__ void __launch_bounds__(kThreadsB) logprobs_bwd_kernel(const LogprobPa
       f[j + 1] = zero ? 0.f : g.y;
     }
     if (v == at_vec) {
+      const float own = at_target();
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (j == at_pos) f[j] += at;
+        if (j == at_pos) f[j] = own;
     }
     st_v4(dv + v, Vec<T>::pack(f));
   };

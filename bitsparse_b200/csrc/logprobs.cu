@@ -54,6 +54,10 @@ struct LogprobParams {
   int32_t *status;
   // backward
   const float *gl, *gh, *ent;
+  // Differences to the maximum are cut off here: p is 0 already, and b times the
+  // cut is finite at the smallest temperatures too (b is up to 1e20 then; 0 times
+  // an infinite product would be NaN).
+  float cut;
   void *dx;
   int64_t ldd;
 };
@@ -620,12 +624,12 @@ __global__ void __launch_bounds__(kThreadsB) logprobs_bwd_kernel(const LogprobPa
   // (Only there: few rows wait for it.)  One thread of a row comes here.
   auto at_target = [&]() {
     if (none || dead) return none ? 0.f : at;
-    const float d = fmaxf(Vec<T>::get(x + target) - m, kFloor), p = ex2(fmaf(d, k, shift));
+    const float d = fmaxf(Vec<T>::get(x + target) - m, P.cut), p = ex2(fmaf(d, k, shift));
     const float logprob = fmaf(d, P.rcp_t, -log_s);
     return fmaf(at, logprob > -0.5f ? -expm1f(logprob) : 1.f - p, p * fmaf(b, d, ah));
   };
   auto grad = [&](float v, int c) {
-    const float d = fmaxf(v - m, kFloor);
+    const float d = fmaxf(v - m, P.cut);
     if (c == target) return at_target();
     return none || dead ? 0.f : ex2(fmaf(d, k, shift)) * fmaf(b, d, a_);
   };
@@ -650,7 +654,7 @@ __global__ void __launch_bounds__(kThreadsB) logprobs_bwd_kernel(const LogprobPa
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
       float2 d = __fadd2_rn(make_float2(f[j], f[j + 1]), minus_m);
-      d = make_float2(fmaxf(d.x, kFloor), fmaxf(d.y, kFloor));
+      d = make_float2(fmaxf(d.x, P.cut), fmaxf(d.y, P.cut));
       const float2 z = __ffma2_rn(d, k2, shift2);
       const float2 g = __fmul2_rn(make_float2(ex2(z.x), ex2(z.y)), __ffma2_rn(b2, d, a2));
       f[j] = zero ? 0.f : g.x;
@@ -758,6 +762,7 @@ extern "C" int bs_token_logprobs_backward(const void *logits, int dtype, int64_t
   LogprobParams P = {};
   P.x = logits; P.target = targets; P.rows = rows; P.V = V; P.ld = ld; P.ignore = ignore_index;
   P.rcp_t = 1.f / temperature; P.stats = const_cast<float *>(stats); P.ent = entropy;
+  P.cut = -256.f / (P.rcp_t * kLog2e);
   P.gl = d_logprobs; P.gh = d_entropy; P.dx = d_logits; P.ldd = ldd;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // a CTA a row (its columns' sums of indices are paid once a row), several

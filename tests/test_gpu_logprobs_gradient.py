@@ -1,9 +1,12 @@
 """GPU: the gradient of token_logprobs where its terms nearly cancel (rows with
-one token that has nearly all of the probability)."""
+one token that has nearly all of the probability) and where they are largest
+(the smallest temperatures, with masked tokens)."""
 import pytest
 import torch
 
 from bitsparse_b200.losses import token_logprobs
+
+from tests.op_util import close
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +82,33 @@ def test_confident_bf16_logits():
     at = d.gather(-1, t.unsqueeze(-1)).squeeze(-1).double()
     want = rest / (1 + rest)
     assert ((at - want).abs() <= (2.0 ** -8 + 2e-5) * want).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("temperature, gh", [(1e-10, 1.0), (1e-10, 1000.0), (1e-8, 1e5)])
+@pytest.mark.parametrize("V, offset", [(1000, None), (1003, None), (1003, 1), (20000, None)])
+def test_masked_tokens_at_small_temperatures(V, offset, temperature, gh, dtype):
+    """Logits as small as the temperature, so that the distribution is an
+    ordinary one; masked tokens get exactly nothing, all others their slope."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = (torch.randn(7, V, generator=g, device="cuda") * 3 * temperature).to(dtype)
+    gone = torch.rand(V, generator=g, device="cuda") < 0.4
+    for fill in (-float("inf"), torch.finfo(dtype).min):
+        y = x.masked_fill(gone, fill)
+        y[3] = fill
+        y[3, 5] = 0.0
+        y = y if offset is None else view(y, offset)
+        t = torch.full((7,), int((~gone).nonzero()[0]), device="cuda")
+        y = y.detach().requires_grad_()
+        r = token_logprobs(y, t, temperature=temperature)
+        w = torch.full((7,), gh, device="cuda")
+        d, = torch.autograd.grad((r.logprobs, r.entropy), y, (w * 0.5, w))
+        z = y.detach().double() / temperature
+        lp = torch.log_softmax(z, -1)
+        p = lp.exp()
+        entropy = torch.special.entr(p)
+        want = gh * (entropy - p * entropy.sum(-1, keepdim=True)) - 0.5 * gh * p
+        want.scatter_add_(-1, t.unsqueeze(-1), 0.5 * w.double().unsqueeze(-1))
+        close(d, want / temperature, "d_logits")
+        keep = torch.arange(7, device="cuda") != 3
+        assert (d[keep][:, gone] == 0).all()

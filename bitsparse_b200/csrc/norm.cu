@@ -81,6 +81,14 @@ Chunks divide(int64_t T, int64_t div_rows, int64_t want) {
 int64_t division(bool gate, int64_t gate_rows, int gate_wide, int64_t T) {
   return gate && gate_wide && gate_rows > 1 ? gate_rows : T;
 }
+// Shifted rows: eight CTAs share a range, which has to be of one gate group, and
+// each has a row of every sum.  For widths of eight, which take this form only
+// where a parameter is off its alignment, no more than the other forms have: the
+// workspace does not know how the tensors lie, and with eight a group it was 113 MB
+// for 4600 x 512 bf16 (4.7 MB) in groups of two.
+bool shares_groups(int64_t groups, int64_t D, int64_t ctas, int64_t most) {
+  return groups < 4 * (ctas / 8) && (D % 8 != 0 || 8 * groups <= most);
+}
 }  // namespace
 }  // namespace bs
 
@@ -125,14 +133,14 @@ extern "C" size_t bs_residual_norm_workspace_bytes(int64_t T, int64_t D, int pos
   int sms = 0;
   if (T <= 0 || D <= 0 || (has_gate && (gate_rows <= 0 || gate_rows > T || T % gate_rows)) ||
       sm_count(&sms) != BS_OK) return 0;
-  // divide() gives at most `want` chunks, or one (shifted rows: eight) for each
-  // of fewer than 4 want groups (shifted: want / 2)
+  // divide() gives at most `want` chunks, or one for each of fewer than 4 want
+  // groups; shifted rows have eight for each while shares_groups()
   const int64_t want = most_ctas(D, sms);
   const int64_t groups = T / division(has_gate, gate_rows, gate_wide, T);
   const bool shifted = T >= kShiftedRows * (int64_t)sms;
   int64_t chunks = shifted || want < T ? want : T;
   if (groups < 4 * want && groups > chunks) chunks = groups;
-  if (shifted && groups < want && 8 * groups > chunks) chunks = 8 * groups;
+  if (shifted && shares_groups(groups, D, want, want) && 8 * groups > chunks) chunks = 8 * groups;
   const int64_t planes = 1 + (post || has_gate ? 1 : 0) + (has_gate ? 1 : 0);
   return (size_t)(planes * chunks * D + (has_gate && !gate_wide ? T : 0)) * sizeof(float);
 }
@@ -185,8 +193,8 @@ extern "C" int bs_residual_norm_backward(
                     (w ? 1 : 0) + (post_w ? 1 : 0), mode, sms);
   };
   BwdPlan plan = plan_of(rows_mode(vec, contiguous, D));
-  // shifted rows: eight CTAs share a range, which has to be of one gate group
-  if (plan.mode == kRowsShifted && (!plan.staged || T / P.div_rows >= 4 * (plan.ctas / 8)))
+  if (plan.mode == kRowsShifted &&
+      (!plan.staged || !shares_groups(T / P.div_rows, D, plan.ctas, most_ctas(D, sms))))
     plan = plan_of(kRowsAny);
   const int share = plan.mode == kRowsShifted ? 8 : 1;
   const Chunks c = divide(T, P.div_rows, plan.ctas / share);

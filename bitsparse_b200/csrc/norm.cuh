@@ -571,9 +571,11 @@ struct RowParam {
   Raw8<T> raw[NV];
   __device__ __forceinline__ void fetch(const Cols &c) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+      raw[v] = {};  // of a thread past the row's end: its zeros are multiplied by this
       if (p && c.first(v) < c.D)
         get_raw(raw[v], static_cast<const uint8_t *>(p) + c.first(v) * (int)sizeof(T));
+    }
   }
   __device__ __forceinline__ void take(float2 (&f)[4], int v, const Cols &) const {
 #pragma unroll

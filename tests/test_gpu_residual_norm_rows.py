@@ -1,5 +1,5 @@
-"""GPU: residual_norm where gate groups divide the rows in every way: results, and
-the workspace that is asked for."""
+"""GPU: residual_norm where a row's last threads have no columns, and where gate
+groups divide the rows in every way."""
 import pytest
 import torch
 
@@ -24,6 +24,28 @@ def check_where_they_are(v, grads):
     want = torch.autograd.grad(exact, list(ref.values()), [g.double() for g in grads])
     for k, a, b in zip(("stream", "normed", *own), (*out, *got), (*exact, *want)):
         close(a, b, k, scale=4.0 if k in own else 1.0)
+
+
+@pytest.mark.parametrize("p_t", [BF16, F32])
+@pytest.mark.parametrize("gate", ["none", "channel", "full"])
+@pytest.mark.parametrize("D", [72, 520, 1032, 1032 + 256, 2056, 2568, 4104, 5128, 7176])
+def test_nan_rows_beside_idle_threads(D, gate, p_t):
+    """Widths that leave threads without columns: every third row is NaN, and
+    nothing of it, nor of anything that such a thread never read, reaches the
+    other rows' outputs and gradients."""
+    T = 1480
+    v, grads = inputs((T,), D, BF16, BF16, p_t, True, gate, seed=D)
+    bad = torch.arange(T, device="cuda") % 3 == 1
+    v["y"][bad] = float("nan")
+    own = {k: t.clone().requires_grad_() for k, t in v.items()}
+    out = residual_norm(own["x"], own["y"], own["weight"], post_norm=True,
+                        post_weight=own["post_weight"], gate=own.get("gate"))
+    names = [k for k in ("x", "y") + (("gate",) if gate == "full" else ())]
+    got = torch.autograd.grad(out, [own[k] for k in names], grads)
+    for t in (*out, *got):
+        assert torch.isnan(t[bad]).any(-1).all() and torch.isfinite(t[~bad]).all()
+    fine = {k: t[~bad] if t.shape[:1] == (T,) and t.dim() == 2 else t for k, t in v.items()}
+    check(fine, tuple(g[~bad] for g in grads), post=True)
 
 
 def workspace(T, D, post, gate_rows, wide=1):

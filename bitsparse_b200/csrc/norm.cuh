@@ -556,6 +556,15 @@ __device__ __forceinline__ void copy_rest(uint8_t *to, const Staged &a, int64_t 
         *reinterpret_cast<uint32_t *>(to + p) = *reinterpret_cast<const uint32_t *>(from + p);
     }
 }
+// Thread 0, where its wait for row `k` of `rows` gave up: the copies of that row
+// and of those requested after it are waited for (with the same limit), so that
+// none lands after the CTA has left.
+__device__ __forceinline__ void drain(uint64_t *full, int k, int rows, int stages) {
+  const int end = k + stages < rows ? k + stages : rows;
+  for (; k < end; ++k)
+    for (uint32_t n = 0; n < kMaxPolls; ++n)
+      if (mbar_try_wait(&full[k % stages], (uint32_t)(k / stages) & 1)) break;
+}
 // Rows near enough to a tensor's ends for that (16 bytes are 8 elements at most).
 __device__ __forceinline__ bool near_end(int64_t row, int64_t rows) {
   return row < 8 || row >= rows - 8;
@@ -649,22 +658,22 @@ __global__ void __launch_bounds__(W == 4 ? 512 : 256, W == 4 ? 1 : 3)
   __syncthreads();
   int stage = 0;
   uint32_t phase = 0;
+  int lost = 0;  // row + 1 whose wait gave up: go on without waiting or copying (results invalid)
   // After a reduction, when every thread has read this stage: the first one for
   // bf16 parameters.  (For fp32 ones that came out slower, 140 against 125 us.)
   auto refill = [&](int k) {
-    if (t == 0 && k + P.stages < rows) {
+    if (t == 0 && !lost && k + P.stages < rows) {
       fence_proxy_async_smem();
       request(k + P.stages, stage);
     }
   };
-  bool lost = false;  // a wait gave up: go on without waiting (the results are invalid)
   for (int k = 0; k < rows; ++k) {
     const int64_t row = blockIdx.x + (int64_t)k * gridDim.x;
     if (!lost) {
       uint32_t n = 0;
       while (!mbar_try_wait(&full[stage], phase) && n < kMaxPolls) ++n;
       if (n == kMaxPolls) {
-        lost = true;
+        lost = k + 1;
         status_or(P.status, BS_STATUS_TIMEOUT);
       }
     }
@@ -770,6 +779,7 @@ __global__ void __launch_bounds__(W == 4 ? 512 : 256, W == 4 ? 1 : 3)
       put8<MODE, true>(static_cast<TY *>(P.h) + row * D, xs[v], v, cols);
     }
   }
+  if (t == 0 && lost) drain(full, lost - 1, rows, P.stages);
 }
 
 // Rows wider than the registers hold: the row is read once for each
@@ -925,7 +935,7 @@ __global__ void __launch_bounds__(GATE == 2 || W == 4 ? 512 : 256, GATE == 2 || 
   __syncthreads();
   int stage = 0;
   uint32_t phase = 0;
-  bool lost = false;  // a wait gave up: go on without waiting (the results are invalid)
+  int lost = 0;  // row + 1 whose wait gave up: go on without waiting or copying (results invalid)
   float r_next = rows > 0 ? P.r_pre[r0] : 0.f;
   float ry_next = POST && rows > 0 ? P.r_post[r0] : 1.f;
   for (int k = 0; k < rows; ++k) {
@@ -957,7 +967,7 @@ __global__ void __launch_bounds__(GATE == 2 || W == 4 ? 512 : 256, GATE == 2 || 
       uint32_t n = 0;
       while (!mbar_try_wait(&full[stage], phase) && n < kMaxPolls) ++n;
       if (n == kMaxPolls) {
-        lost = true;
+        lost = k + 1;
         status_or(P.status, BS_STATUS_TIMEOUT);
       }
     }
@@ -1024,7 +1034,7 @@ __global__ void __launch_bounds__(GATE == 2 || W == 4 ? 512 : 256, GATE == 2 || 
 #pragma unroll
     for (int i = 0; i < NS; ++i) sums[i] = sum2[i].x + sum2[i].y;
     row_sums<NS, true>(sums, buf, turn);
-    if (t == 0 && k + P.stages < rows) {  // every thread has read this stage
+    if (t == 0 && !lost && k + P.stages < rows) {  // every thread has read this stage
       fence_proxy_async_smem();
       request(k + P.stages, stage);
     }
@@ -1097,6 +1107,7 @@ __global__ void __launch_bounds__(GATE == 2 || W == 4 ? 512 : 256, GATE == 2 || 
       }
     }
   }
+  if (t == 0 && lost) drain(full, lost - 1, rows, P.stages);
   const int64_t mine = (int64_t)blockIdx.x * D, plane = P.chunks * (int64_t)D;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {

@@ -13,6 +13,7 @@ import threading
 import ctypes as C
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 
@@ -43,6 +44,16 @@ def ptr(t: torch.Tensor | None) -> int | None:
 def require_cuda(t: torch.Tensor, name: str = "tensor") -> None:
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor (bitsparse_b200 has no CPU path)")
+
+
+def refuse_tangents(*tensors: torch.Tensor | None) -> None:
+    """Forward mode is not implemented: a tangent is refused, not dropped.  (It
+    does not show in requires_grad, by which a call passes autograd by.)"""
+    if getattr(_forward_ad, "_current_level", 0) < 0:  # outside any dual_level()
+        return
+    for t in tensors:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("bitsparse_b200 has no forward-mode derivatives")
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -124,6 +124,7 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, top: int = 0, temperature
         raise ValueError(f"top must lie in 0..{min(MAX_TOP, V)}, not {top}")
     if not 1e-10 <= temperature <= 1e10:
         raise ValueError("temperature must be positive (1e-10 to 1e10)")
+    R.refuse_tangents(logits)
     t = targets.to(torch.int64).contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*_TokenLogprobs.apply(logits, t, top, float(temperature),

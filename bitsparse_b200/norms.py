@@ -238,6 +238,7 @@ def residual_norm(x: Tensor, y: Tensor, weight: Tensor | None = None, *, post_no
             raise TypeError(f"gate must be bfloat16 or float32, not {gate.dtype}")
         gate_rows, wide = _gate_rows(gate.shape, shape[:-1], D)
         gate = gate.contiguous()
+    R.refuse_tangents(x, y, w, pw, gate)
     cfg = (bool(post_norm), gate_rows, wide, _ACTS[gate_act], float(skip_scale),
            float(branch_scale), _check_eps(eps), y_t)
     if torch.is_grad_enabled() and (
@@ -260,6 +261,7 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, *, eps: float = 1e-6,
         raise TypeError(f"no norm of {x.dtype} in {dtype}")
     D = x.shape[-1]
     w = _param(weight, "weight", x.device, D)
+    R.refuse_tangents(x, w)
     cfg = (False, 1, False, 0, 1.0, 1.0, _check_eps(eps), dtype)
     if torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad)):
         return _ResidualNorm.apply(x, None, w, None, None, cfg)

@@ -58,7 +58,7 @@ def _forward(logits, targets, top, temperature, ignore, save):
 
 
 def _grads(ctx, d_lp, d_ent, *_):
-    logits, targets, ent = ctx.saved_tensors
+    logits, targets, ent, stats = ctx.saved_tensors
     n, V, dt, dev = targets.numel(), ctx.shape[-1], logits.dtype, logits.device
     d = torch.empty_like(logits) if logits.shape == ctx.shape and logits.is_contiguous() else \
         logits.new_empty(ctx.shape)
@@ -67,7 +67,7 @@ def _grads(ctx, d_lp, d_ent, *_):
         d_ent = None if d_ent is None else d_ent.contiguous()
         x, ld = _rows(logits, V)
         R.launch(dev, "bs_token_logprobs_backward", x.data_ptr(), _TYPES[dt], n, V, ld,
-                 targets.data_ptr(), ctx.ignore, ctx.temperature, ctx.stats.data_ptr(),
+                 targets.data_ptr(), ctx.ignore, ctx.temperature, stats.data_ptr(),
                  ent.data_ptr(), R.ptr(d_lp), R.ptr(d_ent), d.data_ptr(), V,
                  R.stream_handle(dev))
     return d, None, None, None, None
@@ -83,8 +83,7 @@ class _TokenLogprobs(Function):
                                                      True)
         ctx.set_materialize_grads(False)
         ctx.temperature, ctx.ignore, ctx.shape = temperature, ignore, logits.shape
-        ctx.stats = stats
-        ctx.save_for_backward(x, targets, ent)
+        ctx.save_for_backward(x, targets, ent, stats)
         if top:
             ctx.mark_non_differentiable(top_lp, top_ix)
             return lp, ent, top_lp, top_ix

@@ -165,11 +165,11 @@ def _backward(ds, dh, s, y, w, pw, gate, r, shape, cfg, wants):
 
 
 def _grads(ctx, *grads):
-    s, y, w, pw, gate = ctx.saved_tensors
+    s, y, w, pw, gate, r = ctx.saved_tensors
     ds, dh = grads if len(grads) == 2 else (None, grads[0])
     ds = None if ds is None else ds.contiguous()
     dh = None if dh is None else dh.contiguous()
-    return (*_backward(ds, dh, s, y, w, pw, gate, ctx.r, ctx.shape, ctx.cfg,
+    return (*_backward(ds, dh, s, y, w, pw, gate, r, ctx.shape, ctx.cfg,
                        ctx.needs_input_grad[:5]), None)
 
 
@@ -179,13 +179,14 @@ _grads_once = once_differentiable(_grads)
 class _ResidualNorm(Function):
     @staticmethod
     def forward(ctx, x, y, w, pw, gate, cfg):
-        s, h, ctx.r, x, y = _forward(x, y, w, pw, gate, cfg, True)
+        s, h, r, x, y = _forward(x, y, w, pw, gate, cfg, True)
         ctx.cfg, ctx.shape = cfg, h.shape
         ctx.set_materialize_grads(False)
         # a norm or gate on the branch needs y, and the stream is formed again
         # from x and y; else the stream alone is kept
         branch = cfg[0] or gate is not None
-        ctx.save_for_backward(x if branch or y is None else s, y if branch else None, w, pw, gate)
+        ctx.save_for_backward(x if branch or y is None else s, y if branch else None, w, pw, gate,
+                              r)
         return (s, h) if y is not None else h
 
     @staticmethod

@@ -1,5 +1,6 @@
-"""GPU: residual_norm, rms_norm and token_logprobs under forward mode, which is
-refused, not answered without its tangents."""
+"""GPU: residual_norm, rms_norm and token_logprobs inside autograd's other
+tools: forward mode is refused, not answered without its tangents; what the
+backward needs goes through saved-tensor hooks."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -40,3 +41,27 @@ def test_forward_mode_is_refused(name):
     again = f(v)
     for a, b in zip(each(plain), each(again)):
         assert torch.equal(a, b)
+
+
+def test_saved_tensors_leave_the_gpu():
+    """Under hooks that move what is saved to the host, nothing of the forward
+    but its outputs stays on the device."""
+    rows = 100_000
+    x = torch.randn(rows, 8, device="cuda", requires_grad=True)
+    y = torch.randn(rows, 8, device="cuda", requires_grad=True)
+    t = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    cases = (lambda: residual_norm(x, y, post_norm=True), lambda: rms_norm(x),
+             lambda: token_logprobs(x, t)[:2])
+    for f in cases:
+        f()  # (what the library keeps by itself)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        with torch.autograd.graph.save_on_cpu():
+            out = f()
+        out = each(out)
+        own = sum(o.numel() * o.element_size() + 511 for o in out)
+        held = torch.cuda.memory_allocated() - before
+        assert held <= own  # (rows * 4 bytes of statistics would be 400 KB more)
+        got = torch.autograd.grad([o.sum() for o in out], x)[0]
+        want = torch.autograd.grad([o.sum() for o in each(f())], x)[0]
+        assert torch.equal(got, want)

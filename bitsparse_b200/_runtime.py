@@ -89,11 +89,29 @@ def launch(device: torch.device, name: str, *args) -> None:
         _lib.check(rc, name)
 
 
-def status_word(device: torch.device) -> torch.Tensor:
+class _LibraryWord:
+    """The library's own status word of the current device."""
+
+    def __init__(self):
+        at = C.c_void_p()
+        _lib.call("bs_status_word", C.addressof(at))
+        self._at = at.value
+
+    def data_ptr(self) -> int:
+        return self._at
+
+
+def status_word(device: torch.device) -> torch.Tensor | _LibraryWord:
+    """The device's status word, by its ``data_ptr()``."""
     idx = _index(device)
     s = _status.get(idx)
     if s is not None:
         return s
+    with torch.cuda.device(idx):
+        if torch.cuda.is_current_stream_capturing():
+            # A tensor made here would be the graph's: cleared by every replay.
+            # check_status() reads the library's word too.
+            return _LibraryWord()
     with _lock:
         s = _status.get(idx)
         if s is None:

@@ -595,7 +595,8 @@ __device__ __forceinline__ void scatter_chunk(const uint8_t *stg, uint32_t first
 constexpr int kPipeMaskBytes = kUT * kTileBytes;
 
 // Status word of the reconstruct kernels (bs_unpack has no status argument):
-// BS_STATUS_TIMEOUT when a bounded wait gave up.  Read with bs_unpack_status.
+// BS_STATUS_TIMEOUT when a bounded wait gave up.  Read with bs_unpack_status;
+// bs_status_word gives its address.
 __device__ int32_t g_unpack_status = 0;
 
 // SQ: the ReLU^2 reconstruct of bf16 storage with k = 1 (RELU2_SCALE): each
@@ -1107,6 +1108,18 @@ extern "C" int bs_unpack_relu2_fp8t(const void *vals, const uint8_t *bitmask,
     else unpack_kernel<BS_E5M2, false, 2, false><<<g, kThreads, 0, st>>>(P);
   }
   return launch_err();
+}
+
+extern "C" int bs_status_word(int32_t **word) {
+  if (!word) return BS_ERR_ARG;
+  // finding it may load this library's code, which a strict capture would refuse
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return BS_ERR_LAUNCH;
+  void *at = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&at, g_unpack_status);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  *word = static_cast<int32_t *>(at);
+  return launch_code(e);
 }
 
 extern "C" int bs_unpack_status(int32_t *status_out, int reset) {

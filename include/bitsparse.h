@@ -255,6 +255,11 @@ int bs_fp8_estimate_exact(const float *scale, int fp8_flags, int *out, void *str
  * persistent reconstruct gave up).  Synchronous; reset != 0 clears it. */
 int bs_unpack_status(int32_t *status_out, int reset);
 
+/* Address of that word on the current device, for callers that have no word of
+ * their own to give as `status` (one that is allocated inside a stream capture
+ * would be cleared by every replay).  May be called while a stream captures. */
+int bs_status_word(int32_t **word);
+
 /* In place grad <- bit ? grad : 0 for a bf16 [M, N] gradient (row stride
  * ld).  Replaces mask_with_bitmask_ (lib_sparse/src/triton_operators.py:165-175,
  * lib_sparse/src/triton_kernels.py:249-276). */

@@ -162,24 +162,39 @@ class Muon(torch.optim.Optimizer):
     def _step_shape(self, group, params, rows, cols):
         momentum, lr = group["momentum"], group["lr"]
         narrow = params[0].dtype != torch.float32
-        grads = [p.grad.float() for p in params]
+
+        def batch_of(tensors):
+            return torch.stack([t.reshape(rows, cols) for t in tensors])
+
+        def views(batch):
+            return [t.view(p.shape) for t, p in zip(batch.unbind(), params)]
+
+        grads = [p.grad for p in params]
+        if narrow:
+            batch = batch_of(grads).float()
+            grads = views(batch)
         bufs = self._states(params, "momentum_buffer")
         torch._foreach_mul_(bufs, momentum)
         torch._foreach_add_(bufs, grads)
-        updates = torch._foreach_add(grads, bufs, alpha=momentum) if group["nesterov"] else bufs
-        batch = torch.stack([u.reshape(rows, cols) for u in updates])
+        if group["nesterov"] and narrow:
+            torch._foreach_add_(grads, bufs, alpha=momentum)  # in the batch
+        else:
+            batch = batch_of(torch._foreach_add(grads, bufs, alpha=momentum)
+                             if group["nesterov"] else bufs)
         o = orthogonalize(batch, steps=group["steps"], coefficients=group["coefficients"])
-        values = params
-        if narrow:  # the fp32 values that the parameters are the roundings of
-            values = self._states(params, "remainder")
-            torch._foreach_add_(values, params)
-            for p, v in zip(params, values):
-                v.copy_(torch.where(v.to(p.dtype) == p, v, p))
-        if group["weight_decay"]:
-            torch._foreach_mul_(values, 1 - lr * group["weight_decay"])
-        scale = max(1.0, rows / cols) ** 0.5
-        steps = [v.view(p.shape).float() for p, v in zip(params, o.unbind())]
-        torch._foreach_add_(values, steps, alpha=-lr * scale)
-        if narrow:  # rounded once; the difference is exact
-            torch._foreach_copy_(params, values)
-            torch._foreach_sub_(values, params)
+        decay, rate = 1 - lr * group["weight_decay"], -lr * max(1.0, rows / cols) ** 0.5
+        if not narrow:
+            if decay != 1:
+                torch._foreach_mul_(params, decay)
+            torch._foreach_add_(params, views(o.float()), alpha=rate)
+            return
+        rest = self._states(params, "remainder")
+        own, values = batch_of(params), batch_of(rest)
+        values.add_(own)  # what the parameters are the roundings of
+        torch.where(values.to(own.dtype) == own, values, own, out=values)
+        if decay != 1:
+            values.mul_(decay)
+        values.add_(o, alpha=rate)
+        own.copy_(values)  # rounded once; the difference is exact
+        torch._foreach_copy_(params, views(own))
+        torch._foreach_copy_(rest, views(values.sub_(own)))

@@ -110,11 +110,13 @@ class Muon(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov,
                                       weight_decay=weight_decay, steps=steps,
                                       coefficients=coefficients))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() < 2:
-                    raise ValueError("Muon steps matrices; a parameter has "
-                                     f"{p.dim()} dimension(s)")
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)  # (makes the parameters a list)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                self.param_groups.pop()
+                raise ValueError(f"Muon steps matrices; a parameter has {p.dim()} dimension(s)")
 
     def load_state_dict(self, state_dict):
         """The state is copied, in fp32: the base class would cast it to the

@@ -193,3 +193,13 @@ def test_types_without_a_step_are_refused_before_anything_changes(device):
         with pytest.raises(TypeError):
             opt.step()
         assert not opt.state[params[0]] and torch.equal(params[0], start)
+
+
+def test_added_groups_are_checked_too():
+    opt = Muon([torch.nn.Parameter(torch.zeros(3, 4))])
+    for bad in (torch.zeros(4), torch.zeros(())):
+        with pytest.raises(ValueError):
+            opt.add_param_group({"params": [torch.nn.Parameter(bad)]})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(2, 2))], "lr": 0.5})
+    assert len(opt.param_groups) == 2

@@ -1,6 +1,7 @@
 """GPU: the gradient of token_logprobs where its terms nearly cancel (rows with
 one token that has nearly all of the probability) and where they are largest
-(the smallest temperatures, with masked tokens)."""
+(the smallest temperatures, with masked tokens); the logits of a shifted
+model."""
 import pytest
 import torch
 
@@ -112,3 +113,16 @@ def test_masked_tokens_at_small_temperatures(V, offset, temperature, gh, dtype):
         close(d, want / temperature, "d_logits")
         keep = torch.arange(7, device="cuda") != 3
         assert (d[keep][:, gone] == 0).all()
+
+
+def test_logits_of_a_shifted_model():
+    logits = torch.randn(3, 9, 517, device="cuda", requires_grad=True)
+    tokens = torch.randint(0, 517, (3, 9), device="cuda")
+    lp = token_logprobs(logits[:, :-1], tokens[:, 1:]).logprobs
+    got, = torch.autograd.grad(lp.sum(), logits)
+    ref = logits.detach().double().requires_grad_()
+    want = torch.log_softmax(ref[:, :-1], -1).gather(-1, tokens[:, 1:, None]).squeeze(-1)
+    exact, = torch.autograd.grad(want.sum(), ref)
+    assert (lp.double() - want).abs().max() <= 1e-5
+    assert (got.double() - exact).abs().max() <= 1e-6
+    assert got[:, -1].abs().sum() == 0

@@ -1,5 +1,6 @@
-"""GPU: residual_norm where a row's last threads have no columns, and where gate
-groups divide the rows in every way."""
+"""GPU: residual_norm where a row's last threads have no columns, where gate
+groups divide the rows in every way, and for wide rows with more rows than
+SMs."""
 import pytest
 import torch
 
@@ -75,3 +76,12 @@ def test_workspace_of_gate_groups(groups, rows, D):
     off = {k: torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape) for k, t in v.items()}
     check_where_they_are({**v, "weight": off["weight"]}, grads)
     check_where_they_are(off, grads)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("gate, post", [("none", False), ("none", True), ("channel", True),
+                                        ("batch", True), ("full", True), ("token", False)])
+@pytest.mark.parametrize("D", [8200, 12288, 16385])
+def test_wide_rows_in_number(D, gate, post, dtype):
+    check(*inputs((5, 61), D, dtype, dtype, dtype, post, gate, seed=D), post=post, act="sigmoid",
+          branch=0.5)

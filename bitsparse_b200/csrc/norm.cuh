@@ -859,10 +859,11 @@ __device__ __forceinline__ void chunk_range(const NormParams &P, int64_t b, int6
 // row is taken into registers before its reduction, whose barrier therefore
 // also frees its stage.  bf16 parameters are fetched before the wait for the
 // row, but a norm's on the branch with an element gate, which has no registers
-// for them (16 x 1024 x 4096 bf16, norm and sigmoid gate: 212 us with both
-// parameters read where they are used, 200 as it is, 354 with both fetched early,
-// from spills; norm alone 162 -> 153, no norm at 1024 columns 29 -> 25.  Where
-// HBM binds, as in 16384 x 2048 on an fp32 stream, it cost 94 -> 100 us).
+// for them (16 x 1024 x 4096 bf16: 354 us from spills).  Backward and column sums
+// with the fetch and without: 16384 x 4096 bf16 with a norm 165 and 175 us, with an
+// element gate too 214 and 216, with a channel gate 208 and 228; on an fp32 stream
+// 16384 x 2048 105 both, with a norm 116 and 126; 4096 x 6144 bf16 with a norm and a
+// channel gate, two vectors a thread, 153 and 161 in spite of its spills.
 //
 // GATE: 0 none, 1 an element each (in the stage), 4 the same with a sigmoid, 2
 // columns shared by rows (in registers while the group lasts, its sums too), 3

@@ -35,8 +35,8 @@
 // the others (a look at one, and the proxy fence, take over 1000 clocks), warp
 // 0 loads, warp 1 issues the MMAs, warps 2..9 are the epilogue of the previous
 // tile out of the other half of TMEM (the scheme of gemm.cu).  Stores by TMA:
-// plain stores and the release that has to follow them cost more (24 x 1024 x
-// 1024: 613 us, by TMA 564).
+// with plain stores and the release that has to follow them 24 x 1024 x 1024 took
+// 1.09 times as long.
 #include "common.cuh"
 #include "orthogonal.cuh"
 #include "tcgen05.cuh"
@@ -83,9 +83,9 @@ template <int CG>
 struct OrthCfg {
   static constexpr int T = 128 * CG;
   static constexpr uint32_t COLS = T;  // TMEM columns of an accumulator
-  // 4, 5 and 6 stages measure alike (24 x 1024 x 1024: 605, 613, 624 us; 4096 x
-  // 4096: 1265, 1263, 1248): the main loop takes about 780 clocks for the 512 of
-  // a stage's MMAs because 32 KB a stage come in at 42 bytes a clock, not
+  // 4 and 6 stages measure alike (back to back 24 x 1024 x 1024: 685 and 694 us;
+  // 4096 x 4096: 1324 and 1306): the main loop takes about 780 clocks for the 512
+  // of a stage's MMAs because 32 KB a stage come in at 42 bytes a clock, not
   // because they come late.
   static constexpr int NST = 6;
   static constexpr int EPI = kEpiWarps * 2 * kBoxO;  // a box and a transposed one a warp
@@ -748,10 +748,11 @@ bool set_tiles(OrthParams &P, int64_t T) {
 }
 // CTA pairs on 256 x 256 tiles where those are enough to keep 64 pairs busy in
 // every phase and their ragged edges cost less than the pairs gain; else 128 x
-// 128 tiles.  On whole tiles singles take 1.57 times as long (4096 x 4096: 1843
-// against 1177 us; 24 x 1024 x 1024: 882 against 626), on 24 x 300 x 300, half of
-// whose 256-tiles is edge, 141 against 171 us; with fewer than 64 pair tiles a
-// phase's latency decides (4 x 1024 x 1024: 194 us singles, 219 us pairs).
+// 128 tiles.  Back to back, singles against pairs: on whole tiles 24 x 1024 x 1024
+// 900 and 694 us, 4096 x 4096 1802 and 1306; where pairs compute 1.44 times as much,
+// 24 x 600 x 1300, 585 and 518; at 1.53 times, 24 x 640 x 640 285 and 291, 48 x 520 x
+// 520 555 and 525; above, 24 x 384 x 384 135 and 169, 24 x 300 x 300 132 and 162.  With
+// fewer than 64 pair tiles a phase's latency decides (4 x 1024 x 1024: 191 and 218).
 int run_orth(const OrthMaps &maps, OrthParams &P, cudaStream_t st) {
   if (!set_tiles(P, 128)) return BS_ERR_TOO_LARGE;
   auto products = [&](double tile) {  // of a step, by the tiles' areas

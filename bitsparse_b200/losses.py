@@ -105,7 +105,9 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, top: int = 0, temperature
     are not read: 0, indices -1, no gradient.  Where every logit is -inf, log
     probabilities are -inf and the entropy 0; where one is NaN or +inf, all is
     NaN.  A target outside the vocabulary gives NaN and no gradient, and
-    ``check_status()`` reports it.
+    ``check_status()`` reports it.  Rows may have any one stride; rows that have
+    none, as those of a batch's ``logits[:, :-1]``, are copied first (to ignore
+    each sequence's last position instead reads the logits where they are).
     """
     R.require_cuda(logits, "logits")
     if logits.dtype not in _TYPES:

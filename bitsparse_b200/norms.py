@@ -183,7 +183,9 @@ class _ResidualNorm(Function):
         ctx.cfg, ctx.shape = cfg, h.shape
         ctx.set_materialize_grads(False)
         # a norm or gate on the branch needs y, and the stream is formed again
-        # from x and y; else the stream alone is kept
+        # from x and y.  Else the stream alone is kept, as it was stored: half the
+        # memory and four arrays to read and write in place of five, for a bf16
+        # weight's gradient 2.4e-3 off in 2-norm where its own rounding is 1.7e-3
         branch = cfg[0] or gate is not None
         ctx.save_for_backward(x if branch or y is None else s, y if branch else None, w, pw, gate,
                               r)
